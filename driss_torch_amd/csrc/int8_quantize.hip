@@ -92,7 +92,7 @@ __global__ __launch_bounds__(WAVES == 1 ? kBlock : WAVES * kWave) void int8_rows
   if (t == 0) scale[row] = s.scale;
 }
 
-// Rows that no workgroup holds, and tensors off the vectors' alignment: element by element, twice.
+// Rows that no workgroup holds or that are shorter than a vector, and tensors off the vectors' alignment: element by element, twice.
 template <int IN>
 __global__ __launch_bounds__(kBlock) void int8_rows_any_kernel(const void* __restrict__ x, int64_t cols, uint8_t* __restrict__ q, float* __restrict__ scale) {
   __shared__ uint32_t lds[kBlock / kWave];
@@ -115,7 +115,7 @@ int launch_int8_quantize(const void* x, int64_t rows, int64_t cols, uint8_t* q, 
   constexpr int kV = InTraits<IN>::kVec;
   const int64_t vecs = ceil_div(cols, kV);  // of a row, one with its edges
   const bool base_ok = aligned(x, 16) && aligned(q, IN == DT_F32 ? 4 : 8);
-  if (!base_ok || vecs > 16 * 1024) {
+  if (!int8_rows_in_registers(base_ok, cols, kV)) {
     launcher(int8_rows_any_kernel<IN>, (unsigned)rows, kBlock, 0, stream)(x, cols, q, scale);
     return launch_status();
   }

@@ -7,6 +7,7 @@
 #pragma once
 
 #include "quant_kernels.hpp"
+#include "row_cut.hpp"
 
 namespace dt {
 
@@ -25,31 +26,16 @@ constexpr int kRowsPerBlock = kBlock / kWave;  // one wave per row
 // compiler may put a wait and a copy behind a load, one memory latency more per row: us, fp32 1000 x 1000 3.65 -> 3.17,
 // bf16 2071 x 1952 4.5 -> 4.2.)
 template <int IN, bool EDGES>
-struct RowSpan {
-  static constexpr int kV = InTraits<IN>::kVec, kB = InTraits<IN>::kBytes;
-  int64_t from;    // the vector that the row's first element lies in
-  int64_t vec0;    // first whole vector
-  int nvec;        // whole vectors
-  int skip, tail;  // elements of vector `from` that are the row's before; elements behind the last whole vector
+struct RowSpan : RowCut<InTraits<IN>::kVec, EDGES> {
+  typedef RowCut<InTraits<IN>::kVec, EDGES> Cut;
+  static constexpr int kB = InTraits<IN>::kBytes;
+  using Cut::from;
+  using Cut::skip;
   __amdgpu_buffer_rsrc_t vectors;
   // row, cols: the same for the whole wave
-  __device__ RowSpan(const void* x, int64_t row, int64_t cols) {
-    const uint64_t first = (uint64_t)row * (uint64_t)cols;
-    from = (int64_t)(first / kV);
-    skip = EDGES ? (int)(first % kV) : 0;
-    vec0 = from + (skip != 0);
-    const int64_t rest = cols - (skip ? kV - skip : 0);
-    nvec = (int)((uint64_t)rest / kV);
-    tail = EDGES ? (int)((uint64_t)rest % kV) : 0;
-    vectors = descriptor(x, vec0, nvec * 16);
-  }
+  __device__ RowSpan(const void* x, int64_t row, int64_t cols) : Cut(row, cols) { vectors = descriptor(x, Cut::vec0, Cut::nvec * 16); }
   __device__ u32x4 load(int j) const {  // vector j of the row, or zeros
     return __builtin_amdgcn_raw_buffer_load_b128(vectors, j * 16, 0, kStreaming);
-  }
-  __device__ int edge(int lane_of_row) const {  // the lane's single element, counted from vector `from`; -1: none
-    const int head = skip ? kV - skip : 0;
-    const int at_tail = (int)(vec0 - from + nvec - 1) * kV + lane_of_row;
-    return lane_of_row < head ? skip + lane_of_row : lane_of_row >= kV && lane_of_row < kV + tail ? at_tail : -1;
   }
   __device__ uint32_t load_edge(const void* x, int64_t cols, int edge) const {  // that element as fp32 bits, or zero
     const __amdgpu_buffer_rsrc_t elements = descriptor(x, from, (skip + (int)cols) * kB);

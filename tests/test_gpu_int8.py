@@ -217,3 +217,29 @@ def test_refusals(gpu_device):
 def test_product_of_two_launches(gpu_device, m, n, k):
     """more tiles than CUs: whole rounds of large ones and the columns behind them in smaller ones, with and without shares of K and copies"""
     check_product(*operands(m, n, k, m, gpu_device))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols", range(1, 18))
+def test_quantize_narrow_rows(gpu_device, cols, dtype):
+    """rows that begin and end inside one vector, and those just longer: each has a scale and codes of its own"""
+    g = torch.Generator().manual_seed(cols)
+    for rows in (2, 3, 64, 1031):
+        check_quantize((torch.randn(rows, cols, generator=g) * torch.exp(4 * torch.randn(rows, 1, generator=g))).to(dtype).to(gpu_device))
+
+
+@pytest.mark.parametrize("cols", [1, 3, 7])
+def test_quantize_narrow_rows_write_nothing_else(gpu_device, cols):
+    """codes and scales between words of a pattern, which stay; a row that is not finite leaves its neighbours alone"""
+    rows = 37
+    x = torch.randn(rows, cols, generator=torch.Generator().manual_seed(cols))
+    x[5, cols - 1], x[20, 0] = float("nan"), float("inf")
+    want, scale = quantized(x)
+    x = x.to(gpu_device)
+    q = torch.full((64 + rows * cols + 64,), 85, dtype=torch.int8, device=gpu_device)
+    s = torch.full((16 + rows + 16,), 7.0, device=gpu_device)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert cabi.lib().dt_int8_quantize(x.data_ptr(), cabi.F32, rows, cols, q.data_ptr() + 64, s.data_ptr() + 64, stream) == 0
+    q, s = q.cpu(), s.cpu()
+    assert torch.equal(q[64:-64].view(rows, cols), want) and torch.equal(s[16:-16].nan_to_num(-1.0, -2.0).view(rows, 1), scale.nan_to_num(-1.0, -2.0))
+    assert (q[:64] == 85).all() and (q[-64:] == 85).all() and (s[:16] == 7).all() and (s[-16:] == 7).all()
