@@ -47,6 +47,17 @@ bool elements_aligned(int dtype, std::initializer_list<const void*> tensors) {
   return true;
 }
 
+// No rows: the gradients of what has none of their own are zero
+__global__ __launch_bounds__(256) void norm_zero_kernel(uint16_t* __restrict__ to, int64_t words) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) to[i] = 0;
+}
+int norm_zero(void* to, int dtype, int64_t elements, hipStream_t stream) {
+  if (!to || elements == 0) return DT_OK;
+  const int64_t words = elements * (dtype == DT_F32 ? 2 : 1);
+  launcher(norm_zero_kernel, (unsigned)std::min<int64_t>(ceil_div(words, 256), 4096), 256, 0, stream)(static_cast<uint16_t*>(to), words);
+  return launch_status();
+}
+
 }  // namespace
 }  // namespace dt
 
@@ -78,9 +89,15 @@ extern "C" int dt_norm_backward(int form, const void* d_new_residual, const void
   dt::NormArgs a{new_residual, branch, post_weight, pre_weight, gate, 0, 0, 0, residual_scale, 0.f};
   const int status = dt::norm_args(a, form, dtype, rows, cols, gate, gates);
   if (status != DT_OK) return status;
-  if (rows == 0) return DT_OK;
-  if (cols == 0) return DT_ERR_EMPTY;
   const bool post = form & dt::kNormPost, pre = form & dt::kNormPre;
+  if (rows == 0) {
+    if (!dt::elements_aligned(dtype, {d_post_weight, d_pre_weight, d_gate})) return DT_ERR_MISALIGNED;
+    const hipStream_t s = dt::as_hip(stream);
+    if (const int st = dt::norm_zero(post ? d_post_weight : nullptr, dtype, cols, s)) return st;
+    if (const int st = dt::norm_zero(pre ? d_pre_weight : nullptr, dtype, cols, s)) return st;
+    return dt::norm_zero(gate ? d_gate : nullptr, dtype, gates * cols, s);
+  }
+  if (cols == 0) return DT_ERR_EMPTY;
   if ((post && (!branch || !post_weight || !inverse_y || !d_branch || !d_post_weight)) || (pre && (!new_residual || !pre_weight || !inverse_r || !d_residual || !d_pre_weight)) ||
       (gate && !d_gate))
     return DT_ERR_NULL_POINTER;

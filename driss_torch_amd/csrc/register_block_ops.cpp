@@ -269,11 +269,6 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> norm_backward(const std::opti
   Tensor d_residual = new_output(pre ? new_residual.sizes() : kNothing, type, new_residual), d_branch = new_output(post ? new_residual.sizes() : kNothing, type, new_residual);
   Tensor d_post = new_output({post ? s.cols : 0}, type, new_residual), d_pre = new_output({pre ? s.cols : 0}, type, new_residual);
   Tensor d_gate = new_output(gate ? gate->sizes() : kNothing, type, new_residual);
-  if (s.rows == 0) {
-    d_post.zero_();
-    d_pre.zero_();
-    return {d_residual, d_branch, d_post, d_pre, d_gate};
-  }
   const Tensor dr = contiguous_or_none(d_new_residual), dn = contiguous_or_none(d_normed), r = new_residual.contiguous(), y = contiguous_or_none(branch),
                p = contiguous_or_none(post_weight), w = contiguous_or_none(pre_weight);
   const Workspace ws(dt_norm_backward_workspace_bytes(s.form, s.gates, s.dtype, s.rows, s.cols), new_residual);

@@ -361,7 +361,8 @@ DT_API int dt_norm_forward(int form, const void* residual, const void* branch, c
 /* The gradients for d_new_residual and d_normed (NULL: zero; only those of the form's results count).
  * new_residual: the forward's result (form DT_NORM_PRE: its residual).  With DT_NORM_POST alone the
  * residual's gradient is d_new_residual itself and d_residual is not written.  Sums over rows are
- * taken in fp32, always in the same order.                                                 */
+ * taken in fp32, always in the same order; with rows == 0 the weights' and the gate's gradients are
+ * written as zeros (those that are not NULL), and no workspace is needed.                  */
 DT_API size_t dt_norm_backward_workspace_bytes(int form, int64_t gates, int dtype, int64_t rows,
                                                int64_t cols);
 DT_API int dt_norm_backward(int form, const void* d_new_residual, const void* d_normed,

@@ -5,6 +5,7 @@ import torch
 
 import driss_torch as d
 import feed_forward_reference as ref
+from driss_torch_amd import cabi
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float32]
@@ -195,3 +196,36 @@ def test_long_rows(gpu_device, rows, cols, gates, dtype):
 def test_long_rows_of_one_norm(gpu_device, rows, cols, gates, form, dtype):
     v = inputs(rows, cols, 0 if form == "pre" else gates, dtype, rows + cols, gpu_device, form)
     check(run(v, form), reference(v), (rows, cols, gates, form))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("form", ["pre", "post", "post_pre"])
+@pytest.mark.parametrize("gate_shape", [None, (40,), (1, 40), (3, 1, 40)])
+def test_no_rows_with_a_gate(gpu_device, gate_shape, form, dtype):
+    """a rank that is given no tokens: gradients of weights and gate are zero, whatever the memory held that they are made in"""
+    if form == "pre" and gate_shape:
+        return
+    v = inputs(6, 40, 0, dtype, 0, gpu_device, form)
+    v = {k: t[:0] if t is not None and t.dim() == 2 else t for k, t in v.items()}
+    v["gate"] = torch.ones(gate_shape, dtype=dtype, device=gpu_device) if gate_shape else None
+    names = [k for k in ("post_weight", "pre_weight", "gate") if v[k] is not None]
+    for _ in range(3):
+        held = [torch.full((n,), float("nan"), dtype=dtype, device=gpu_device) for n in (40, 120) for _ in range(8)]
+        del held
+        got = run(v, form)
+        for k in names:
+            assert got["d_" + k].shape == v[k].shape and got["d_" + k].eq(0).all(), k
+
+
+@pytest.mark.parametrize("dtype,code", [(torch.bfloat16, cabi.BF16), (torch.float32, cabi.F32)])
+def test_no_rows_through_the_c_interface(gpu_device, dtype, code):
+    """zeros in what is not NULL, nothing behind it, no workspace"""
+    p, cols, gates = torch.ones(40, dtype=dtype, device=gpu_device), 33, 2
+    stream = torch.cuda.current_stream().cuda_stream
+    for given in ((1, 1, 1), (1, 0, 1), (0, 1, 0)):
+        out = [torch.full((n + 3,), 5.0, dtype=dtype, device=gpu_device) for n in (cols, cols, gates * cols)]
+        d_post, d_pre, d_gate = (t.data_ptr() if there else None for t, there in zip(out, given))
+        at = p.data_ptr()
+        assert cabi.lib().dt_norm_backward(3, at, at, at, at, at, at, at, gates, code, 0, cols, 1.0, None, None, None, None, d_post, d_pre, d_gate, None, 0, stream) == 0
+        for t, there in zip(out, given):
+            assert (t[:-3] == (0 if there else 5)).all() and (t[-3:] == 5).all()
