@@ -155,7 +155,7 @@ def norm_forward_meta(residual, branch, post_weight, pre_weight, gate, residual_
             residual.new_empty((rows if pre and keep else 0,), dtype=torch.float32))
 
 
-def norm_backward_meta(d_new_residual, d_normed, new_residual, branch, post_weight, pre_weight, gate, inverse_y, inverse_r, residual_scale):
+def norm_backward_meta(d_new_residual, d_normed, new_residual, branch, post_weight, pre_weight, gate, inverse_y, inverse_r, residual_scale, from_residual=False):
     r, post, pre = new_residual, branch is not None, pre_weight is not None
     return (r.new_empty(r.shape if pre else (0,)), r.new_empty(r.shape if post else (0,)), r.new_empty((r.shape[-1] if post else 0,)),
             r.new_empty((r.shape[-1] if pre else 0,)), r.new_empty(gate.shape if gate is not None else (0,)))

@@ -79,6 +79,7 @@ extern "C" int dt_norm_forward(int form, const void* residual, const void* branc
 
 extern "C" size_t dt_norm_backward_workspace_bytes(int form, int64_t gates, int dtype, int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0 || gates < 0 || (gates > 0 && rows % gates)) return 0;
+  form &= ~(int)DT_NORM_FROM_RESIDUAL;
   return (size_t)dt::norm_units(dtype, rows, cols, gates > 0 ? rows / gates : rows).units * (size_t)cols * sizeof(float) * (form == dt::kNormPostPre ? 2 : 1);
 }
 
@@ -86,7 +87,10 @@ extern "C" int dt_norm_backward(int form, const void* d_new_residual, const void
                                 const void* pre_weight, const void* gate, int64_t gates, int dtype, int64_t rows, int64_t cols, float residual_scale,
                                 const float* inverse_y, const float* inverse_r, void* d_residual, void* d_branch, void* d_post_weight, void* d_pre_weight, void* d_gate,
                                 void* workspace, size_t workspace_bytes, dt_stream_t stream) {
-  dt::NormArgs a{new_residual, branch, post_weight, pre_weight, gate, 0, 0, 0, residual_scale, 0.f};
+  const bool rebuild = form & DT_NORM_FROM_RESIDUAL;
+  form &= ~(int)DT_NORM_FROM_RESIDUAL;
+  if (rebuild && (form != dt::kNormPostPre || dtype != DT_BF16)) return DT_ERR_INVALID_MODE;
+  dt::NormArgs a{new_residual, branch, post_weight, pre_weight, gate, 0, 0, 0, residual_scale, 0.f, rebuild};
   const int status = dt::norm_args(a, form, dtype, rows, cols, gate, gates);
   if (status != DT_OK) return status;
   const bool post = form & dt::kNormPost, pre = form & dt::kNormPre;

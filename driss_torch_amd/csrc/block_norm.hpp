@@ -115,6 +115,7 @@ struct NormArgs {
   int cols;
   int64_t rows_per_gate;  // of a row of the gate
   float scale, eps;
+  bool rebuild;  // gradients of both norms, bf16: `residual` is the forward's r, of which r' is built again
 };
 
 // kTeams teams of WAVES waves in a workgroup: four where a wave is a team, so that a workgroup is never one wave
@@ -318,7 +319,8 @@ __global__ __launch_bounds__(kNormTeams<WAVES>* WAVES* kWave) void norm_backward
   auto weight_n = [&](int u, float (&f)[V::kVec]) __attribute__((always_inline)) { V::unpack(HOLD ? held_n[HOLD ? u : 0] : Row::template load<false>(a.pre_weight, 0, a.cols, t + u * kThreads), f); };
   auto gate = [&](int u, float (&f)[V::kVec]) __attribute__((always_inline)) { V::unpack(HOLD ? held_gate[HOLD ? u : 0] : Row::template load<false>(a.gate, gate_row, a.cols, t + u * kThreads), f); };
   // what of the rows is on its way: gradients of both results, r' where its norm needs it, y.  A row stays packed as it came and is unpacked again
-  // behind each sum: half the registers of bf16.
+  // behind each sum: half the registers of bf16.  r' of bf16 rows is the exception: it is not what the forward rounded and stored but, from r, y and y's
+  // inverse, the same fp32 value whose norm the forward took, bit for bit, and stays in 32 bits over the sum (in place of dr', which stays packed).
   u32x4 next_dr[NV], next_dn[NV], next_r[NV], next_y[NV];
   float next_iy = 0.f, next_ir = 0.f;
   auto fetch = [&](int64_t at) __attribute__((always_inline)) {
@@ -339,10 +341,12 @@ __global__ __launch_bounds__(kNormTeams<WAVES>* WAVES* kWave) void norm_backward
   };
   const float inverse_cols = 1.0f / (float)a.cols;
   constexpr bool AHEAD = HOLD || SUMS_IN_LDS;
+  constexpr bool REBUILD = IN == DT_BF16 && FORM == kNormPostPre;
   if (AHEAD && row < end) fetch(row);
   while (row < end) {
     if constexpr (!AHEAD) fetch(row);
-    u32x4 raw_dn[NV], raw_r[NV], raw_y[NV];
+    u32x4 raw_dn[NV], raw_r[NV], raw_y[NV], raw_dr[NV];
+    float r_new[REBUILD ? NV : 1][V::kVec];
     float d[NV][V::kVec];  // the residual's gradient
     const float iy = next_iy, ir = next_ir;
 #pragma unroll
@@ -352,7 +356,8 @@ __global__ __launch_bounds__(kNormTeams<WAVES>* WAVES* kWave) void norm_backward
         raw_r[u] = next_r[u];
       }
       if constexpr (POST) {
-        V::unpack(next_dr[u], d[u]);
+        raw_dr[u] = next_dr[u];
+        if constexpr (!PRE) V::unpack(raw_dr[u], d[u]);
         raw_y[u] = next_y[u];
       }
     }
@@ -364,16 +369,45 @@ __global__ __launch_bounds__(kNormTeams<WAVES>* WAVES* kWave) void norm_backward
         if constexpr (HOLD) {
 #pragma unroll
           for (int u = 0; u < NV; ++u) held_gate[u] = Row::template load<false>(a.gate, gate_row, a.cols, t + u * kThreads);
+          // (waited for here: where every row uses it, a wait for it would be one for the next row's loads as well; both norms with all gradients,
+          // 16384 x 8192 bf16 527 us and 499)
+          __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
         }
       }
     }
+    if constexpr (REBUILD) {
+      const float scale = iy * a.scale;
+#pragma unroll
+      for (int u = 0; u < NV; ++u) {
+        V::unpack(raw_r[u], r_new[u]);
+        if (!a.rebuild) continue;
+        float y[V::kVec], p[V::kVec], g[V::kVec];
+        V::unpack(raw_y[u], y);
+        weight_p(u, p);
+        if (a.gate) gate(u, g);
+#pragma unroll
+        for (int i = 0; i < V::kVec; ++i) {
+          float z = y[i] * scale * p[i];
+          if (a.gate) z *= g[i];
+          r_new[u][i] += z;
+        }
+      }
+    }
+    auto row_r = [&](int u, float (&f)[V::kVec]) __attribute__((always_inline)) {
+      if constexpr (REBUILD) {
+#pragma unroll
+        for (int i = 0; i < V::kVec; ++i) f[i] = r_new[u][i];
+      } else {
+        V::unpack(raw_r[u], f);
+      }
+    };
     if constexpr (PRE) {
       float sum = 0.f;
 #pragma unroll
       for (int u = 0; u < NV; ++u) {
         float dn[V::kVec], r[V::kVec], w[V::kVec];
         V::unpack(raw_dn[u], dn);
-        V::unpack(raw_r[u], r);
+        row_r(u, r);
         weight_n(u, w);
 #pragma unroll
         for (int i = 0; i < V::kVec; ++i) {
@@ -387,8 +421,9 @@ __global__ __launch_bounds__(kNormTeams<WAVES>* WAVES* kWave) void norm_backward
       for (int u = 0; u < NV; ++u) {
         float dn[V::kVec], r[V::kVec], w[V::kVec];
         V::unpack(raw_dn[u], dn);
-        V::unpack(raw_r[u], r);
+        row_r(u, r);
         weight_n(u, w);
+        if constexpr (POST) V::unpack(raw_dr[u], d[u]);
 #pragma unroll
         for (int i = 0; i < V::kVec; ++i) {
           const float through = ir * (dn[i] * w[i] - r[i] * ir * mean);

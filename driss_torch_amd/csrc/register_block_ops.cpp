@@ -251,13 +251,16 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> norm_forward(const Tensor& residual, 
 }
 
 // (d_residual, d_branch, d_post_weight, d_pre_weight, d_gate): what the form does not have is empty, and so is d_residual of a norm behind the
-// block alone, where it is d_new_residual
+// block alone, where it is d_new_residual.  from_residual: new_residual is the forward's residual, of which the operator builds it again in fp32
+// (bf16, both norms)
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> norm_backward(const std::optional<Tensor>& d_new_residual, const std::optional<Tensor>& d_normed, const Tensor& new_residual,
                                                                  const std::optional<Tensor>& branch, const std::optional<Tensor>& post_weight,
                                                                  const std::optional<Tensor>& pre_weight, const std::optional<Tensor>& gate, const Tensor& inverse_y,
-                                                                 const Tensor& inverse_r, double residual_scale) {
+                                                                 const Tensor& inverse_r, double residual_scale, bool from_residual) {
   const NormShape s(new_residual, branch, post_weight, pre_weight, gate);
   const bool post = s.form & DT_NORM_POST, pre = s.form & DT_NORM_PRE;
+  TORCH_CHECK(!from_residual || (post && pre && s.dtype == DT_BF16), "from_residual is for both norms in bfloat16");
+  const int form = s.form | (from_residual ? DT_NORM_FROM_RESIDUAL : 0);
   for (const auto* d : {&d_new_residual, &d_normed}) {
     if (!*d) continue;
     s.check(**d, new_residual, "a gradient");
@@ -271,8 +274,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> norm_backward(const std::opti
   Tensor d_gate = new_output(gate ? gate->sizes() : kNothing, type, new_residual);
   const Tensor dr = contiguous_or_none(d_new_residual), dn = contiguous_or_none(d_normed), r = new_residual.contiguous(), y = contiguous_or_none(branch),
                p = contiguous_or_none(post_weight), w = contiguous_or_none(pre_weight);
-  const Workspace ws(dt_norm_backward_workspace_bytes(s.form, s.gates, s.dtype, s.rows, s.cols), new_residual);
-  check_status(dt_norm_backward(s.form, data_or_null(dr), data_or_null(dn), r.data_ptr(), data_or_null(y), data_or_null(p), data_or_null(w), data_or_null(s.gate), s.gates, s.dtype,
+  const Workspace ws(dt_norm_backward_workspace_bytes(form, s.gates, s.dtype, s.rows, s.cols), new_residual);
+  check_status(dt_norm_backward(form, data_or_null(dr), data_or_null(dn), r.data_ptr(), data_or_null(y), data_or_null(p), data_or_null(w), data_or_null(s.gate), s.gates, s.dtype,
                                 s.rows, s.cols, (float)residual_scale, post ? inverse_y.data_ptr<float>() : nullptr, pre ? inverse_r.data_ptr<float>() : nullptr,
                                 pre ? d_residual.data_ptr() : nullptr, post ? d_branch.data_ptr() : nullptr, post ? d_post.data_ptr() : nullptr, pre ? d_pre.data_ptr() : nullptr,
                                 s.gates ? d_gate.data_ptr() : nullptr, ws.data(), ws.bytes, ctx.stream),
@@ -344,7 +347,10 @@ struct BlockNorm : Function<BlockNorm> {
     auto [new_residual, normed, iy, ir] = op.call(residual, branch, post_weight, pre_weight, gate, residual_scale, eps, true);
     ctx->set_materialize_grads(false);
     const Tensor none;
-    ctx->save_for_backward({branch ? new_residual : residual, branch.value_or(none), post_weight.value_or(none), pre_weight.value_or(none), gate.value_or(none), iy, ir});
+    // of both norms in bf16 the gradients take the new residual as the second norm did, before its rounding, and build it again
+    const bool from_residual = branch && pre_weight && residual.scalar_type() == at::kBFloat16;
+    ctx->saved_data["from_residual"] = from_residual;
+    ctx->save_for_backward({branch && !from_residual ? new_residual : residual, branch.value_or(none), post_weight.value_or(none), pre_weight.value_or(none), gate.value_or(none), iy, ir});
     ctx->saved_data["residual_scale"] = residual_scale;
     if (!branch) return {normed};
     if (!pre_weight) return {new_residual};
@@ -360,8 +366,9 @@ struct BlockNorm : Function<BlockNorm> {
     static auto op =
         operator_of<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>(const std::optional<Tensor>&, const std::optional<Tensor>&, const Tensor&, const std::optional<Tensor>&,
                                                                        const std::optional<Tensor>&, const std::optional<Tensor>&, const std::optional<Tensor>&, const Tensor&,
-                                                                       const Tensor&, double)>("DrissTorch::norm_backward");
-    auto [dr, dy, dp, dw, dg] = op.call(some(d_new), some(d_normed), v[0], some(v[1]), some(v[2]), some(v[3]), some(v[4]), v[5], v[6], ctx->saved_data["residual_scale"].toDouble());
+                                                                       const Tensor&, double, bool)>("DrissTorch::norm_backward");
+    auto [dr, dy, dp, dw, dg] = op.call(some(d_new), some(d_normed), v[0], some(v[1]), some(v[2]), some(v[3]), some(v[4]), v[5], v[6], ctx->saved_data["residual_scale"].toDouble(),
+                                      ctx->saved_data["from_residual"].toBool());
     out[0] = pre ? dr : d_new;
     if (post) {
       out[1] = dy;
@@ -439,6 +446,6 @@ TORCH_LIBRARY_FRAGMENT(DrissTorch, m) {
   m.impl("norm_forward", DispatchKey::CUDA, TORCH_FN(driss_torch::norm_forward));
   m.def(
       "norm_backward(Tensor? d_new_residual, Tensor? d_normed, Tensor new_residual, Tensor? branch, Tensor? post_weight, Tensor? pre_weight, Tensor? gate, "
-      "Tensor inverse_y, Tensor inverse_r, float residual_scale) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+      "Tensor inverse_y, Tensor inverse_r, float residual_scale, bool from_residual=False) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.impl("norm_backward", DispatchKey::CUDA, TORCH_FN(driss_torch::norm_backward));
 }

@@ -352,14 +352,16 @@ DT_API int dt_gated_linear_backward(const void* dh, const void* x, const void* w
  * DT_BF16); gate [gates, cols] with rows % gates == 0, each of its rows for rows / gates rows in
  * turn, or NULL with gates == 0.  inverse_y, inverse_r [rows]: 1 / sqrt(...) of both norms, for
  * dt_norm_backward; may be NULL.  cols <= 32768.                                           */
-enum dt_norm_form { DT_NORM_POST = 1, DT_NORM_PRE = 2, DT_NORM_POST_PRE = 3 };
+enum dt_norm_form { DT_NORM_POST = 1, DT_NORM_PRE = 2, DT_NORM_POST_PRE = 3, DT_NORM_FROM_RESIDUAL = 4 };
 DT_API int dt_norm_forward(int form, const void* residual, const void* branch, const void* post_weight,
                            const void* pre_weight, const void* gate, int64_t gates, int dtype,
                            int64_t rows, int64_t cols, float residual_scale, float eps,
                            void* new_residual, void* normed, float* inverse_y, float* inverse_r,
                            dt_stream_t stream);
 /* The gradients for d_new_residual and d_normed (NULL: zero; only those of the form's results count).
- * new_residual: the forward's result (form DT_NORM_PRE: its residual).  With DT_NORM_POST alone the
+ * new_residual: the forward's result (form DT_NORM_PRE: its residual).  With form DT_NORM_POST_PRE |
+ * DT_NORM_FROM_RESIDUAL, for DT_BF16 alone, it is the forward's residual, of which new_residual is built
+ * again in fp32, as the forward's second norm took it before its rounding to bf16.  With DT_NORM_POST alone the
  * residual's gradient is d_new_residual itself and d_residual is not written.  Sums over rows are
  * taken in fp32, always in the same order; with rows == 0 the weights' and the gate's gradients are
  * written as zeros (those that are not NULL), and no workspace is needed.                  */

@@ -145,3 +145,12 @@ def test_reference_gradients_of_the_norms(gates):
     names = ["d_residual", "d_branch", "d_post_weight", "d_pre_weight"] + (["d_gate"] if gates else [])
     for name, want in zip(names, torch.autograd.grad([stream, normed], leaves, [dr, dn])):
         assert torch.allclose(got[name][0], want, rtol=1e-11, atol=1e-12), name
+
+
+def test_new_residual_built_again_is_of_both_norms_in_bf16():
+    L, p = cabi.lib(), 0x1000  # never dereferenced
+    backward = lambda form, dtype, room: L.dt_norm_backward(form, p, p, p, p, p, p, p, 2, dtype, 64, 100, 1.0, p, p, p, p, p, p, p, p, room, None)  # noqa: E731
+    need = L.dt_norm_backward_workspace_bytes(7, 2, cabi.BF16, 64, 100)
+    assert need == L.dt_norm_backward_workspace_bytes(3, 2, cabi.BF16, 64, 100)
+    assert backward(7, cabi.BF16, need - 1) == 5 and backward(7, cabi.F32, need) == 6 and backward(5, cabi.BF16, need) == 6 and backward(6, cabi.BF16, need) == 6
+    assert backward(4, cabi.BF16, need) == 6 and L.dt_norm_forward(7, p, p, p, p, None, 0, cabi.BF16, 4, 8, 1.0, 1e-6, p, p, None, None, None) == 6

@@ -229,3 +229,42 @@ def test_no_rows_through_the_c_interface(gpu_device, dtype, code):
         assert cabi.lib().dt_norm_backward(3, at, at, at, at, at, at, at, gates, code, 0, cols, 1.0, None, None, None, None, d_post, d_pre, d_gate, None, 0, stream) == 0
         for t, there in zip(out, given):
             assert (t[:-3] == (0 if there else 5)).all() and (t[-3:] == 5).all()
+
+
+@pytest.mark.parametrize("rows,cols,gates", [(5, 40, 1), (64, 1001, 2), (300, 520, 0), (700, 256, 350), (9, 4096, 9), (520, 9224, 1), (30, 12290, 30), (40, 16384, 4), (3, 20000, 0)])
+def test_bf16_gradients_take_the_new_residual_before_its_rounding(gpu_device, rows, cols, gates):
+    """bounds as for fp32 tensors of the same values, which hold no rounding of the new residual, and one rounding of each result"""
+    v = inputs(rows, cols, gates, torch.bfloat16, rows * 3 + cols, gpu_device)
+    got = run(v, "post_pre")
+    want = reference({k: None if t is None else t.float() for k, t in v.items()})
+    for k, (value, bound) in want.items():
+        ref.assert_within(got[k], value, bound + ref.R * (value.abs() + bound), (k, rows, cols, gates))
+
+
+def test_gradients_from_the_new_residual(gpu_device):
+    """the operator that takes the new residual itself: in fp32 the only form, in bf16 with its rounding"""
+    for dtype in DTYPES:
+        v = inputs(50, 264, 2, dtype, 3, gpu_device)
+        r, n, iy, ir = d.ops.norm_forward(*(v[k] for k in ("residual", "branch", "post_weight", "pre_weight", "gate")), 0.7, EPS, True)
+        rest = (v["branch"], v["post_weight"], v["pre_weight"], v["gate"], iy, ir, 0.7)
+        names = ("d_residual", "d_branch", "d_post_weight", "d_pre_weight", "d_gate")
+        got = dict(zip(names, d.ops.norm_backward(v["d_residual"], v["d_normed"], r, *rest)))
+        check(got, {k: t for k, t in reference(v).items() if k in names}, dtype)
+    with pytest.raises(RuntimeError, match="from_residual"):
+        d.ops.norm_backward(v["d_residual"], v["d_normed"], v["residual"], *rest, True)
+
+
+def test_saved_tensors_are_the_callers(gpu_device):
+    """what the gradients read may not change before they are taken; a bf16 result may"""
+    v = inputs(20, 64, 1, torch.bfloat16, 3, gpu_device)
+    want = run(v, "post_pre")
+    leaves = {**v, **{k: v[k].clone().requires_grad_() for k in ("branch", "post_weight")}}
+    out = call(leaves, "post_pre")
+    with torch.no_grad():
+        out["residual"].zero_()
+    got = torch.autograd.grad([out["residual"], out["normed"]], [leaves["branch"]], [v["d_residual"], v["d_normed"]])[0]
+    assert torch.equal(got, want["d_branch"])
+    out = call(leaves, "post_pre")
+    leaves["residual"].add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad([out["residual"], out["normed"]], [leaves["branch"]], [v["d_residual"], v["d_normed"]])
