@@ -311,6 +311,10 @@ bool any_grad(std::initializer_list<const Tensor*> tensors) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// There is no forward-mode rule: a tangent is refused, with or without gradients beside it, rather than dropped
+void reverse_mode_only(const char* name, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors) TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), name, " has no forward-mode derivative (jvp)");
+}
 void first_order_only(const char* name) { TORCH_CHECK(!at::GradMode::is_enabled(), name, " has no gradient of its gradient (create_graph)"); }
 std::optional<Tensor> some(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 // a gradient as the operator wants it: of the input's dtype, which autograd has seen to
@@ -381,12 +385,14 @@ struct BlockNorm : Function<BlockNorm> {
 };
 
 Tensor gated_linear_autograd(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, std::string_view activation) {
+  reverse_mode_only("gated_linear", {&x, &w_gate, &w_up});
   if (any_grad({&x, &w_gate, &w_up})) return GatedLinear::apply(x, w_gate, w_up, std::string(activation));
   at::AutoDispatchBelowADInplaceOrView below;
   static auto op = operator_of<Tensor(const Tensor&, const Tensor&, const Tensor&, std::string_view)>("DrissTorch::gated_linear");
   return op.call(x, w_gate, w_up, activation);
 }
 Tensor pre_norm_autograd(const Tensor& x, const Tensor& weight, double eps) {
+  reverse_mode_only("a block norm", {&x, &weight});
   if (any_grad({&x, &weight})) return BlockNorm::apply(x, std::optional<Tensor>(), std::optional<Tensor>(), std::optional<Tensor>(weight), std::optional<Tensor>(), 1.0, eps)[0];
   at::AutoDispatchBelowADInplaceOrView below;
   static auto op = operator_of<Tensor(const Tensor&, const Tensor&, double)>("DrissTorch::pre_norm");
@@ -394,6 +400,7 @@ Tensor pre_norm_autograd(const Tensor& x, const Tensor& weight, double eps) {
 }
 Tensor post_norm_autograd(const Tensor& residual, const Tensor& branch, const Tensor& weight, const std::optional<Tensor>& gate, double residual_scale, double eps) {
   const Tensor g = gate.value_or(Tensor());
+  reverse_mode_only("a block norm", {&residual, &branch, &weight, &g});
   if (any_grad({&residual, &branch, &weight, &g})) return BlockNorm::apply(residual, std::optional<Tensor>(branch), std::optional<Tensor>(weight), std::optional<Tensor>(), gate, residual_scale, eps)[0];
   at::AutoDispatchBelowADInplaceOrView below;
   static auto op = operator_of<Tensor(const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&, double, double)>("DrissTorch::post_norm");
@@ -402,6 +409,7 @@ Tensor post_norm_autograd(const Tensor& residual, const Tensor& branch, const Te
 std::tuple<Tensor, Tensor> post_pre_norm_autograd(const Tensor& residual, const Tensor& branch, const Tensor& post_weight, const Tensor& pre_weight, const std::optional<Tensor>& gate,
                                                   double residual_scale, double eps) {
   const Tensor g = gate.value_or(Tensor());
+  reverse_mode_only("a block norm", {&residual, &branch, &post_weight, &pre_weight, &g});
   if (any_grad({&residual, &branch, &post_weight, &pre_weight, &g})) {
     const auto out = BlockNorm::apply(residual, std::optional<Tensor>(branch), std::optional<Tensor>(post_weight), std::optional<Tensor>(pre_weight), gate, residual_scale, eps);
     return {out[0], out[1]};

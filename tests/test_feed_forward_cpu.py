@@ -154,3 +154,25 @@ def test_new_residual_built_again_is_of_both_norms_in_bf16():
     assert need == L.dt_norm_backward_workspace_bytes(3, 2, cabi.BF16, 64, 100)
     assert backward(7, cabi.BF16, need - 1) == 5 and backward(7, cabi.F32, need) == 6 and backward(5, cabi.BF16, need) == 6 and backward(6, cabi.BF16, need) == 6
     assert backward(4, cabi.BF16, need) == 6 and L.dt_norm_forward(7, p, p, p, p, None, 0, cabi.BF16, 4, 8, 1.0, 1e-6, p, p, None, None, None) == 6
+
+
+TRAINED = {"gated_linear": 3, "pre_norm": 2, "post_norm": 4, "post_pre_norm": 5}
+
+
+@pytest.mark.parametrize("no_grad", [False, True])
+@pytest.mark.parametrize("name,of", [(name, of) for name, n in TRAINED.items() for of in range(n)])
+def test_a_tangent_is_refused(name, of, no_grad):
+    """forward-mode derivatives there are none: a dual tensor or torch.func.jvp raises, of whichever input, with gradients recorded or not"""
+    with FakeTensorMode():
+        x, w, p = (torch.empty(s, dtype=torch.bfloat16, device="cuda") for s in ((4, 16), (8, 16), (16,)))
+        args = list({"gated_linear": (x, w, w), "pre_norm": (x, p), "post_norm": (x, x, p, p), "post_pre_norm": (x, x, p, p, p)}[name])
+        call = lambda v: getattr(d, name)(*args[:of], v, *args[of + 1:])  # noqa: E731
+        if name == "post_pre_norm" and of == 4:
+            call = lambda v: d.post_pre_norm(*args[:4], gate=v)  # noqa: E731
+        with torch.set_grad_enabled(not no_grad):
+            call(args[of])
+            with torch.autograd.forward_ad.dual_level():
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(torch.autograd.forward_ad.make_dual(args[of], torch.empty_like(args[of])))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.func.jvp(call, (args[of],), (torch.empty_like(args[of]),))
