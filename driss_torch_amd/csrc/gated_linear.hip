@@ -118,9 +118,6 @@ int gated_shape(int64_t T, int64_t D, int64_t F, int64_t ldx, int64_t ldg, int64
   if (T < 0 || D < 0 || F < 0 || T > 0x3FFFFFFFll || D > kGatedMostWidth || F > kGatedMostWidth || ldx < D || ldg < D || ldu < D) return DT_ERR_INVALID_SHAPE;
   return act < kSilu || act > kGeluTanh ? DT_ERR_INVALID_MODE : DT_OK;
 }
-MmPlan gated_forward_plan(int64_t T, int64_t D, int64_t F) { return T > kMmRowsMost ? mm_plan_for(T, 2 * F, 1, ceil_div(D, 64), false) : MmPlan{}; }
-MmPlan gated_dx_plan(int64_t T, int64_t D, int64_t F) { return mm_plan_for(T, D, 1, 2 * ceil_div(F, 64), true); }
-MmPlan gated_dw_plan(int64_t T, int64_t D, int64_t F) { return mm_plan_for(F, D, 2, ceil_div(T, 64), true); }
 
 // the three operands of the projections as their rows lie
 struct GatedRows {
@@ -128,20 +125,43 @@ struct GatedRows {
   GatedRows(const void* x_, const void* wg_, const void* wu_, int64_t T, int64_t D, int64_t F, int64_t ldx, int64_t ldg, int64_t ldu)
       : x{(const uint8_t*)x_, T, D * 2, ldx * 2}, wg{(const uint8_t*)wg_, F, D * 2, ldg * 2}, wu{(const uint8_t*)wu_, F, D * 2, ldu * 2} {}
   // for dx, where K runs through one weight and then the other: rows of both the same distance apart
-  GatedRows& chained() {
+  void chained() {
     if (wg.whole_words() != wu.whole_words() || (wg.whole_words() && wg.ld != wu.ld)) wg.copy = wu.copy = true;
-    return *this;
   }
   size_t packed_bytes() const { return x.packed_bytes() + wg.packed_bytes() + wu.packed_bytes(); }
 };
-size_t slopes_bytes(int64_t T, int64_t F) { return (size_t)(2 * T * ceil_div(F, 8) * 16); }
+
+// A call's operands and plans, made once: the knobs that a plan reads may change at any time, and what is checked has to be what is launched.
+struct GatedForwardCall {
+  GatedRows rows;
+  MmPlan plan{};  // of more than kMmRowsMost rows
+  size_t sums = 0;
+  GatedForwardCall(const void* x, const void* wg, const void* wu, int64_t T, int64_t D, int64_t F, int64_t ldx, int64_t ldg, int64_t ldu) : rows(x, wg, wu, T, D, F, ldx, ldg, ldu) {
+    if (T <= kMmRowsMost) return;
+    plan = mm_plan_for(T, 2 * F, 1, ceil_div(D, 64), false);
+    sums = mm_sums_bytes(plan, T, 2 * F, 1);
+  }
+  size_t workspace_bytes() const { return plan.tiles ? sums + rows.packed_bytes() : 0; }
+};
+struct GatedBackwardCall {
+  GatedRows rows;
+  MmPlan dx, dw;
+  size_t slopes, sums;  // dg and du; the sums of K's shares, of one product after the other
+  GatedBackwardCall(const void* x, const void* wg, const void* wu, int64_t T, int64_t D, int64_t F, int64_t ldx, int64_t ldg, int64_t ldu)
+      : rows(x, wg, wu, T, D, F, ldx, ldg, ldu), dx(mm_plan_for(T, D, 1, 2 * ceil_div(F, 64), true)), dw(mm_plan_for(F, D, 2, ceil_div(T, 64), true)) {
+    rows.chained();
+    slopes = (size_t)(2 * T * ceil_div(F, 8) * 16);
+    sums = std::max(mm_sums_bytes(dx, T, D, 1), mm_sums_bytes(dw, F, D, 2));
+  }
+  size_t workspace_bytes() const { return slopes + sums + rows.packed_bytes(); }
+};
 
 }  // namespace
 }  // namespace dt
 
 extern "C" size_t dt_gated_linear_workspace_bytes(const void* x, const void* w_gate, const void* w_up, int64_t T, int64_t D, int64_t F, int64_t ldx, int64_t ldg, int64_t ldu) {
-  if (T <= dt::kMmRowsMost || D <= 0 || F <= 0) return 0;
-  return dt::GatedRows(x, w_gate, w_up, T, D, F, ldx, ldg, ldu).packed_bytes() + dt::mm_sums_bytes(dt::gated_forward_plan(T, D, F), T, 2 * F, 1);
+  if (T <= 0 || D <= 0 || F <= 0) return 0;
+  return dt::GatedForwardCall(x, w_gate, w_up, T, D, F, ldx, ldg, ldu).workspace_bytes();
 }
 
 extern "C" int dt_gated_linear(const void* x, const void* w_gate, const void* w_up, int64_t T, int64_t D, int64_t F, int64_t ldx, int64_t ldg, int64_t ldu, int act,
@@ -161,15 +181,15 @@ extern "C" int dt_gated_linear(const void* x, const void* w_gate, const void* w_
     if (const int st = dt::mm_zero(g, T, 2 * F, 2 * F, s)) return st;  // (words of two)
     return dt::mm_zero(u, T, 2 * F, 2 * F, s);
   }
-  const dt::GatedRows rows(x, w_gate, w_up, T, D, F, ldx, ldg, ldu);
-  const dt::MmPlan plan = dt::gated_forward_plan(T, D, F);
+  const dt::GatedForwardCall call(x, w_gate, w_up, T, D, F, ldx, ldg, ldu);
+  const dt::GatedRows& rows = call.rows;
+  const dt::MmPlan& plan = call.plan;
   if (!plan.tiles) {
     const dt::MmRowsArgs args{rows.x.p, {rows.wg.p, rows.wu.p}, T > 1 ? rows.x.ld : D * 2, {F > 1 ? rows.wg.ld : D * 2, F > 1 ? rows.wu.ld : D * 2}, (int)T, (int)F, (int)D, 0};
     return dt::launch_mm_rows<dt::Bf16Product, true>(args, rows.packed_bytes() == 0, dt::GatedRowsStore{ho, go, uo, F, act}, s);
   }
-  const size_t need = dt_gated_linear_workspace_bytes(x, w_gate, w_up, T, D, F, ldx, ldg, ldu);
-  if (need > 0 && (!workspace || workspace_bytes < need)) return DT_ERR_WORKSPACE;
-  dt::MmPacking packed(static_cast<uint8_t*>(workspace) + dt::mm_sums_bytes(plan, T, 2 * F, 1));
+  if (const size_t need = call.workspace_bytes(); need > 0 && (!workspace || workspace_bytes < need)) return DT_ERR_WORKSPACE;
+  dt::MmPacking packed(static_cast<uint8_t*>(workspace) + call.sums);
   const dt::MmRows rx = packed(rows.x), rg = packed(rows.wg), ru = packed(rows.wu);
   if (const int st = packed.launch(s)) return st;
   const int k = (int)(dt::ceil_div(D, 2) * 2);  // (what a copy is padded with is zero)
@@ -181,8 +201,7 @@ extern "C" int dt_gated_linear(const void* x, const void* w_gate, const void* w_
 
 extern "C" size_t dt_gated_linear_backward_workspace_bytes(const void* x, const void* w_gate, const void* w_up, int64_t T, int64_t D, int64_t F, int64_t ldx, int64_t ldg, int64_t ldu) {
   if (T <= 0 || D <= 0 || F <= 0) return 0;
-  return dt::GatedRows(x, w_gate, w_up, T, D, F, ldx, ldg, ldu).chained().packed_bytes() + dt::slopes_bytes(T, F) +
-         std::max(dt::mm_sums_bytes(dt::gated_dx_plan(T, D, F), T, D, 1), dt::mm_sums_bytes(dt::gated_dw_plan(T, D, F), F, D, 2));
+  return dt::GatedBackwardCall(x, w_gate, w_up, T, D, F, ldx, ldg, ldu).workspace_bytes();
 }
 
 extern "C" int dt_gated_linear_backward(const void* dh, const void* x, const void* w_gate, const void* w_up, const void* g, const void* u, int64_t T, int64_t D, int64_t F,
@@ -201,15 +220,14 @@ extern "C" int dt_gated_linear_backward(const void* dh, const void* x, const voi
     if (const int st = dt::mm_zero(dw_gate, F, D, D, s)) return st;
     return dt::mm_zero(dw_up, F, D, D, s);
   }
-  if (!workspace || workspace_bytes < dt_gated_linear_backward_workspace_bytes(x, w_gate, w_up, T, D, F, ldx, ldg, ldu)) return DT_ERR_WORKSPACE;
+  const dt::GatedBackwardCall call(x, w_gate, w_up, T, D, F, ldx, ldg, ldu);
+  if (!workspace || workspace_bytes < call.workspace_bytes()) return DT_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int chunks = (int)dt::ceil_div(F, 8);
-  uint8_t *const dg = ws, *const du = ws + dt::slopes_bytes(T, F) / 2;
-  ws += dt::slopes_bytes(T, F);
-  // the sums of K's shares, of one product after the other
-  const dt::MmPlan dx_plan = dt::gated_dx_plan(T, D, F), dw_plan = dt::gated_dw_plan(T, D, F);
+  uint8_t *const dg = ws, *const du = ws + call.slopes / 2;
+  ws += call.slopes;
   void* const sums = ws;
-  ws += std::max(dt::mm_sums_bytes(dx_plan, T, D, 1), dt::mm_sums_bytes(dw_plan, F, D, 2));
+  ws += call.sums;
   {
     const unsigned gx = (unsigned)dt::ceil_div(chunks, 256), gy = (unsigned)(T < 32768 ? T : 32768);
     const uint16_t* pdh = (const uint16_t*)dh;
@@ -220,7 +238,7 @@ extern "C" int dt_gated_linear_backward(const void* dh, const void* x, const voi
     void* at[] = {&pdh, &pg, &pu, &rows, &f, &a, &pdg, &pdu};
     (void)hipLaunchKernel(reinterpret_cast<const void*>(dt::gated_slopes_kernel), dim3(gx, gy), dim3(256), at, 0, s);
   }
-  const dt::GatedRows rows = dt::GatedRows(x, w_gate, w_up, T, D, F, ldx, ldg, ldu).chained();
+  const dt::GatedRows& rows = call.rows;
   const int64_t ldd = (int64_t)chunks * 16;
   dt::MmPacking packed(ws);
   dt::MmRows rg{}, ru{}, rx{};
@@ -229,12 +247,12 @@ extern "C" int dt_gated_linear_backward(const void* dh, const void* x, const voi
   if (const int st = packed.launch(s)) return st;
   if (dx) {
     const dt::MmTileArgs args{{dg, du}, {rg.p, ru.p}, ldd, {rg.ld, ru.ld}, (int)T, (int)D, chunks * 8, (int)F, 0, 0};
-    const int st = dt::launch_mm<dt::Bf16Product, dt::kAlong, dt::kAcross, dt::kMmChain>(args, dx_plan, sums, dt::Bf16Tile{{(uint16_t*)dx, nullptr}, D, (int)T, (int)D}, s);
+    const int st = dt::launch_mm<dt::Bf16Product, dt::kAlong, dt::kAcross, dt::kMmChain>(args, call.dx, sums, dt::Bf16Tile{{(uint16_t*)dx, nullptr}, D, (int)T, (int)D}, s);
     if (st != DT_OK) return st;
   }
   if (dw_gate) {
     const dt::MmTileArgs args{{dg, du}, {rx.p, nullptr}, ldd, {rx.ld, 0}, (int)F, (int)D, (int)T, (int)T, 0, 0};
-    const int st = dt::launch_mm<dt::Bf16Product, dt::kAcross, dt::kAcross, dt::kMmStack>(args, dw_plan, sums, dt::Bf16Tile{{(uint16_t*)dw_gate, (uint16_t*)dw_up}, D, (int)F, (int)D}, s);
+    const int st = dt::launch_mm<dt::Bf16Product, dt::kAcross, dt::kAcross, dt::kMmStack>(args, call.dw, sums, dt::Bf16Tile{{(uint16_t*)dw_gate, (uint16_t*)dw_up}, D, (int)F, (int)D}, s);
     if (st != DT_OK) return st;
   }
   return dt::launch_status();
