@@ -169,6 +169,20 @@ std::tuple<Tensor, Tensor, Tensor> gated_linear_backward(const Tensor& dh, const
 
 // ---------------------------------------------------------------------------- block norms
 namespace {
+// Whether the gate's shape broadcasts to the residual's and would by that give its rows to other rows than equal shares in turn do: a dimension of the
+// residual that the gate has, behind one that it has not
+bool broadcasts_otherwise(const Tensor& gate, const Tensor& residual) {
+  const int64_t missing = residual.dim() - gate.dim();
+  if (missing < 0) return false;
+  bool shared = false, otherwise = false;
+  for (int64_t i = 0; i + 1 < residual.dim(); ++i) {
+    const int64_t rows = residual.size(i), own = i < missing ? 1 : gate.size(i - missing);
+    if (own != 1 && own != rows) return false;
+    if (own != rows) shared = true;
+    else if (own != 1 && shared) otherwise = true;
+  }
+  return otherwise;
+}
 struct NormShape {
   int form = 0, dtype;
   int64_t rows, cols, gates = 0;
@@ -198,6 +212,9 @@ struct NormShape {
       TORCH_CHECK(branch.has_value(), "a gate needs a branch");
       check(*gate_in, residual, "gate");
       TORCH_CHECK(gate_in->dim() >= 1 && gate_in->size(-1) == cols && gate_in->numel() > 0, "gate must have rows of ", cols, " elements, but got ", gate_in->sizes());
+      TORCH_CHECK((gate_in->dim() == 2 && gate_in->size(0) == residual.size(0)) || !broadcasts_otherwise(*gate_in, residual), "gate ", gate_in->sizes(), " with a residual ",
+                  residual.sizes(), ": its rows stand for equal shares of the residual's rows in turn, one per sequence ([B, 1, C]) or one per row; one per position, as broadcasting "
+                  "would have it, has to be expanded to the residual's shape");
       gate = gate_in->reshape({-1, cols}).contiguous();
       gates = gate.size(0);
       TORCH_CHECK(rows % gates == 0, "the gate's ", gates, " rows must divide the residual's ", rows);

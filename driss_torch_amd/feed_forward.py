@@ -49,7 +49,9 @@ def post_norm(residual: Tensor, branch: Tensor, weight: Tensor, gate: Optional[T
     ``residual + residual_scale * gate * (weight * branch / sqrt(mean(branch^2) + eps))``.
 
     residual, branch: [..., C]; gate: [C] or [..., C], whose rows are taken by equal shares of the residual's rows in
-    turn: one for all rows, one per sequence (``[B, C]`` or ``[B, 1, C]`` with residual [B, T, C]), or one per row."""
+    turn: one for all rows, one per sequence (``[B, C]``, of whatever T, or ``[B, 1, C]`` with residual [B, T, C]), or one
+    per row.  A shape that broadcasts to the residual's in another way (``[T, C]`` or ``[1, T, C]``, a row per
+    position) is refused: expand it."""
     return _ops.post_norm(residual, branch, weight, gate, residual_scale, eps)
 
 

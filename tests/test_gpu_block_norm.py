@@ -268,3 +268,30 @@ def test_saved_tensors_are_the_callers(gpu_device):
     leaves["residual"].add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad([out["residual"], out["normed"]], [leaves["branch"]], [v["d_residual"], v["d_normed"]])
+
+
+@pytest.mark.parametrize("shape,gate_shape", [((3, 4, 40), (4, 40)), ((3, 4, 40), (1, 4, 40)), ((2, 3, 4, 40), (2, 1, 4, 40)), ((2, 3, 4, 40), (3, 1, 40)), ((2, 3, 4, 40), (3, 4, 40)),
+                                              ((2, 3, 4, 40), (4, 40)), ((2, 3, 4, 40), (1, 3, 4, 40))])
+def test_a_gate_per_position_is_refused(gpu_device, shape, gate_shape):
+    """shapes whose rows broadcasting would give to other rows than equal shares in turn do; expanded they are taken as they are meant"""
+    v = inputs(1, 40, 0, torch.float32, 1, gpu_device)
+    r, y = (torch.randn(shape, device=gpu_device) for _ in range(2))
+    gate = torch.randn(gate_shape, device=gpu_device)
+    for bad in (lambda: d.post_norm(r, y, v["post_weight"], gate), lambda: d.post_pre_norm(r, y, v["post_weight"], v["pre_weight"], gate)):
+        with pytest.raises(RuntimeError, match="expanded to the residual's shape"):
+            bad()
+    got = d.post_norm(r, y, v["post_weight"], gate.expand(shape), 0.7, EPS)
+    want, bound = ref.norms(r, y, v["post_weight"], None, gate.expand(shape), 0.7, EPS)["residual"]
+    ref.assert_within(got, want, bound)
+
+
+@pytest.mark.parametrize("shape,gate_shape", [((3, 4, 40), (40,)), ((3, 4, 40), (1, 1, 40)), ((3, 4, 40), (3, 40)), ((3, 4, 40), (3, 1, 40)), ((3, 4, 40), (3, 4, 40)), ((4, 4, 40), (4, 40)),
+                                              ((3, 4, 40), (12, 40)), ((3, 4, 40), (6, 40)), ((1, 4, 40), (4, 40)), ((3, 1, 40), (3, 40)), ((2, 3, 4, 40), (2, 3, 1, 40)),
+                                              ((2, 3, 4, 40), (2, 1, 1, 40)), ((2, 3, 4, 40), (2, 40)), ((1, 3, 4, 40), (3, 1, 40)), ((12, 40), (4, 1, 40)), ((1, 1, 40), (1, 40))])
+def test_gates_of_equal_shares(gpu_device, shape, gate_shape):
+    """every shape whose meaning is plain, of whatever number of dimensions"""
+    v = inputs(1, 40, 0, torch.float32, 1, gpu_device)
+    r, y = (torch.randn(shape, device=gpu_device) for _ in range(2))
+    gate = torch.randn(gate_shape, device=gpu_device)
+    want, bound = ref.norms(r, y, v["post_weight"], None, gate, 0.7, EPS)["residual"]
+    ref.assert_within(d.post_norm(r, y, v["post_weight"], gate, 0.7, EPS), want, bound)
