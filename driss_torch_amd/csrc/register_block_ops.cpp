@@ -211,13 +211,13 @@ struct NormShape {
     if (gate_in) {
       TORCH_CHECK(branch.has_value(), "a gate needs a branch");
       check(*gate_in, residual, "gate");
-      TORCH_CHECK(gate_in->dim() >= 1 && gate_in->size(-1) == cols && gate_in->numel() > 0, "gate must have rows of ", cols, " elements, but got ", gate_in->sizes());
+      TORCH_CHECK(gate_in->dim() >= 1 && gate_in->size(-1) == cols && (gate_in->numel() > 0 || rows == 0), "gate must have rows of ", cols, " elements, but got ", gate_in->sizes());
       TORCH_CHECK((gate_in->dim() == 2 && gate_in->size(0) == residual.size(0)) || !broadcasts_otherwise(*gate_in, residual), "gate ", gate_in->sizes(), " with a residual ",
                   residual.sizes(), ": its rows stand for equal shares of the residual's rows in turn, one per sequence ([B, 1, C]) or one per row; one per position, as broadcasting "
                   "would have it, has to be expanded to the residual's shape");
       gate = gate_in->reshape({-1, cols}).contiguous();
       gates = gate.size(0);
-      TORCH_CHECK(rows % gates == 0, "the gate's ", gates, " rows must divide the residual's ", rows);
+      TORCH_CHECK(gates == 0 || rows % gates == 0, "the gate's ", gates, " rows must divide the residual's ", rows);
     }
   }
   void check(const Tensor& t, const Tensor& residual, const char* name) const {
@@ -292,7 +292,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> norm_backward(const std::opti
   const Tensor dr = contiguous_or_none(d_new_residual), dn = contiguous_or_none(d_normed), r = new_residual.contiguous(), y = contiguous_or_none(branch),
                p = contiguous_or_none(post_weight), w = contiguous_or_none(pre_weight);
   const Workspace ws(dt_norm_backward_workspace_bytes(form, s.gates, s.dtype, s.rows, s.cols), new_residual);
-  check_status(dt_norm_backward(form, data_or_null(dr), data_or_null(dn), r.data_ptr(), data_or_null(y), data_or_null(p), data_or_null(w), data_or_null(s.gate), s.gates, s.dtype,
+  check_status(dt_norm_backward(form, data_or_null(dr), data_or_null(dn), r.data_ptr(), data_or_null(y), data_or_null(p), data_or_null(w), s.gates ? s.gate.data_ptr() : nullptr, s.gates, s.dtype,
                                 s.rows, s.cols, (float)residual_scale, post ? inverse_y.data_ptr<float>() : nullptr, pre ? inverse_r.data_ptr<float>() : nullptr,
                                 pre ? d_residual.data_ptr() : nullptr, post ? d_branch.data_ptr() : nullptr, post ? d_post.data_ptr() : nullptr, pre ? d_pre.data_ptr() : nullptr,
                                 s.gates ? d_gate.data_ptr() : nullptr, ws.data(), ws.bytes, ctx.stream),

@@ -295,3 +295,19 @@ def test_gates_of_equal_shares(gpu_device, shape, gate_shape):
     gate = torch.randn(gate_shape, device=gpu_device)
     want, bound = ref.norms(r, y, v["post_weight"], None, gate, 0.7, EPS)["residual"]
     ref.assert_within(d.post_norm(r, y, v["post_weight"], gate, 0.7, EPS), want, bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,gate_shape", [((0, 5, 40), (0, 1, 40)), ((0, 5, 40), (0, 40)), ((0, 5, 40), (0, 5, 40)), ((0, 40), (0, 40)), ((3, 0, 40), (3, 1, 40)), ((3, 0, 40), (3, 0, 40))])
+def test_an_empty_batch_with_its_gate(gpu_device, shape, gate_shape, dtype):
+    """a gate row per sequence where there are no sequences, or sequences without rows"""
+    v = inputs(1, 40, 0, dtype, 1, gpu_device)
+    p, w = v["post_weight"].requires_grad_(), v["pre_weight"].requires_grad_()
+    r, y = (torch.zeros(shape, dtype=dtype, device=gpu_device, requires_grad=True) for _ in range(2))
+    gate = torch.ones(gate_shape, dtype=dtype, device=gpu_device, requires_grad=True)
+    new, normed = d.post_pre_norm(r, y, p, w, gate)
+    assert new.shape == normed.shape == shape and d.post_norm(r, y, p, gate).shape == shape
+    grads = torch.autograd.grad([new, normed], [r, y, p, w, gate], [torch.zeros_like(new), torch.zeros_like(normed)])
+    assert all(g.shape == t.shape and not g.any() for g, t in zip(grads, (r, y, p, w, gate)))
+    with pytest.raises(RuntimeError, match="gate must have rows"):
+        d.post_norm(torch.zeros(2, 40, dtype=dtype, device=gpu_device), torch.zeros(2, 40, dtype=dtype, device=gpu_device), p, torch.zeros(0, 40, dtype=dtype, device=gpu_device))
