@@ -67,7 +67,9 @@ __device__ __forceinline__ void act_and_slope(float g, int act, float& value, fl
   } else {
     const float s = gelu_tanh_gate(g);
     value = g * s;
-    slope = s + g * s * (1.0f - s) * (1.59576912160573071f + 3.0f * 0.0713548162726009f * g * g);
+    // (s is 0 or 1 from |g| = 11 on: what stands beside it there is kept from overflowing, 0 times infinity)
+    const float c = __builtin_amdgcn_fmed3f(g, -16.0f, 16.0f);
+    slope = s + c * s * (1.0f - s) * (1.59576912160573071f + 3.0f * 0.0713548162726009f * c * c);
   }
 }
 

@@ -221,3 +221,26 @@ def test_two_launches(gpu_device, t, dim, f):
     grads = torch.autograd.grad(d.gated_linear(*leaves), leaves, dh)
     for g, (name, (want, bound)) in zip(grads, ref.gated_grads(dh, x, wg, wu, "silu").items()):
         ref.assert_within(g, want, bound, (name, t, dim, f))
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("t", [2, 40, 300])
+def test_gradients_where_squares_overflow(gpu_device, t, act):
+    """gates of +-2^66, whose squares are no fp32 numbers: activations and slopes are at their limits, g and 1 above zero, 0 and 0 below.  Every sum has one
+    term, a product of powers of two, and half the rows have a gate of either sign."""
+    dim, f = 16, 8
+    x, wg, wu = (torch.zeros(n, dim, dtype=torch.bfloat16, device=gpu_device) for n in (t, f, f))
+    x[::2, 0], x[1::2, 0], x[:, 1] = 2.0**66, -(2.0**66), 1.0
+    wg[:, 0], wu[:, 1] = 1.0, 0.5
+    leaves = [v.requires_grad_() for v in (x, wg, wu)]
+    h = d.gated_linear(*leaves, act)
+    assert (h[::2] == 2.0**65).all() and (h[1::2] == 0).all()
+    dh = torch.zeros_like(h)
+    dh[0, 0] = dh[1, 1] = 1.0
+    dx, dg, du = torch.autograd.grad(h, leaves, dh)
+    want = torch.zeros_like(x)
+    want[0, 0], want[0, 1] = 0.5, 2.0**65  # u times the slope 1, times the weight 1; the activation times the weight 0.5
+    assert torch.equal(dx, want)
+    want_g, want_u = torch.zeros_like(wg), torch.zeros_like(wu)
+    want_g[0, 0], want_g[0, 1], want_u[0, 0], want_u[0, 1] = 2.0**65, 0.5, float("inf"), 2.0**66  # (2^132 is past bf16)
+    assert torch.equal(dg, want_g) and torch.equal(du, want_u)
