@@ -111,7 +111,7 @@ __global__ __launch_bounds__(kBlock) void int8_rows_any_kernel(const void* __res
 }
 
 template <int IN>
-int launch_int8_quantize(const void* x, int64_t rows, int64_t cols, uint8_t* q, float* scale, hipStream_t stream) {
+int launch_int8_rows(const void* x, int64_t rows, int64_t cols, uint8_t* q, float* scale, hipStream_t stream) {
   constexpr int kV = InTraits<IN>::kVec;
   const int64_t vecs = ceil_div(cols, kV);  // of a row, one with its edges
   const bool base_ok = aligned(x, 16) && aligned(q, IN == DT_F32 ? 4 : 8);
@@ -136,6 +136,17 @@ int launch_int8_quantize(const void* x, int64_t rows, int64_t cols, uint8_t* q, 
   else DT_INT8_ROWS(16, 16);
 #undef DT_INT8_ROWS
   return launch_status();
+}
+
+// A launch has fewer than 2^32 threads: as many rows at a time as workgroups of 1024 may be, from rows on that lie as the first one does
+constexpr int64_t kInt8MostRows = 1 << 21;
+template <int IN>
+int launch_int8_quantize(const void* x, int64_t rows, int64_t cols, uint8_t* q, float* scale, hipStream_t stream) {
+  for (int64_t row = 0; row < rows; row += kInt8MostRows) {
+    const uint8_t* const from = static_cast<const uint8_t*>(x) + row * cols * InTraits<IN>::kBytes;
+    if (const int st = launch_int8_rows<IN>(from, std::min(rows - row, kInt8MostRows), cols, q + row * cols, scale + row, stream)) return st;
+  }
+  return DT_OK;
 }
 
 }  // namespace

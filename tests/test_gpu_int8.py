@@ -243,3 +243,19 @@ def test_quantize_narrow_rows_write_nothing_else(gpu_device, cols):
     q, s = q.cpu(), s.cpu()
     assert torch.equal(q[64:-64].view(rows, cols), want) and torch.equal(s[16:-16].nan_to_num(-1.0, -2.0).view(rows, 1), scale.nan_to_num(-1.0, -2.0))
     assert (q[:64] == 85).all() and (q[-64:] == 85).all() and (s[:16] == 7).all() and (s[-16:] == 7).all()
+
+
+@pytest.mark.parametrize("rows,cols,dtype", [((1 << 26) + 5, 8, torch.bfloat16), ((1 << 24) + 3, 3, torch.float32), ((1 << 21) + 9, 1030, torch.bfloat16)])
+def test_quantize_many_rows(gpu_device, rows, cols, dtype):
+    """more rows than one launch has threads for, and tensors of more than 2^31 elements: 1021 rows over and over"""
+    period = 1021
+    g = torch.Generator().manual_seed(cols)
+    block = (torch.randn(period, cols, generator=g) * torch.exp(4 * torch.randn(period, 1, generator=g))).to(dtype)
+    x = torch.empty(rows, cols, dtype=dtype, device=gpu_device)
+    whole = rows // period * period
+    x[:whole].view(-1, period, cols).copy_(block.to(gpu_device))
+    x[whole:] = block[:rows - whole].to(gpu_device)
+    q, scale = d.int8_quantize(x)
+    want, ws = (t.to(gpu_device) for t in quantized(block))
+    for got, of in ((q, want), (scale, ws)):
+        assert bool((got[:whole].view(-1, period, of.shape[1]) == of).all()) and torch.equal(got[whole:], of[:rows - whole])
