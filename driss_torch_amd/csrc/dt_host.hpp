@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <utility>
 
 #include "driss_torch_hip.h"
 
@@ -126,7 +127,9 @@ inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_
 inline int64_t ceil_div(int64_t a, int64_t b) { return a / b + (a % b != 0); }  // src/include/utils.h:37-39
 
 // launcher(kernel, grid, block, lds, stream)(arguments...): what kernel<<<grid, block, lds, stream>>>(arguments...) does, without its detour by a
-// call configuration that is stored and fetched again, 2.38 against 2.60 us of the host per launch.  A failure is the last error (launch_status).
+// call configuration that is stored and fetched again, 2.38 against 2.60 us of the host per launch.  A failure is the last error (launch_status), and so is
+// a launch of 2^32 threads or more, which the runtime would cut short without one.
+inline thread_local bool g_launch_too_large = false;
 template <typename... P>
 struct Launcher {
   void (*kernel)(P...);
@@ -135,7 +138,8 @@ struct Launcher {
   hipStream_t stream;
   void operator()(P... arguments) const {
     void* at[] = {&arguments...};
-    (void)hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(grid), dim3(block), at, lds, stream);
+    if ((uint64_t)grid * block > 0xFFFFFFFFull) g_launch_too_large = true;
+    else (void)hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(grid), dim3(block), at, lds, stream);
   }
 };
 template <typename... P>
@@ -143,7 +147,10 @@ inline Launcher<P...> launcher(void (*kernel)(P...), unsigned grid, unsigned blo
   return {kernel, grid, block, lds, stream};
 }
 
-inline int launch_status() { return hipGetLastError() == hipSuccess ? DT_OK : DT_ERR_LAUNCH; }
+inline int launch_status() {
+  const bool too_large = std::exchange(g_launch_too_large, false);
+  return hipGetLastError() == hipSuccess && !too_large ? DT_OK : DT_ERR_LAUNCH;
+}
 
 inline hipStream_t as_hip(dt_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 

@@ -38,7 +38,7 @@ enum dt_status {
   DT_ERR_MISALIGNED = 4,      /* pointer alignment requirement not met */
   DT_ERR_WORKSPACE = 5,       /* workspace missing or too small */
   DT_ERR_INVALID_MODE = 6,    /* round_mode / axis / layout code out of range */
-  DT_ERR_LAUNCH = 7,          /* hipGetLastError() after the launch was not hipSuccess */
+  DT_ERR_LAUNCH = 7,          /* hipGetLastError() after the launch was not hipSuccess, or it had 2^32 threads or more */
   DT_ERR_EMPTY = 8,           /* reduction over zero elements */
   DT_ERR_RESIDENT_GAVE_UP = 9,/* an EARLIER per-tensor dynamic quantization on this device gave up waiting for
                                  the whole chip and wrote NaN outputs (see dt_dynamic_scaled_quant); nothing

@@ -33,7 +33,7 @@ static int read_knob(Knob k) {
 
 static std::map<const void*, std::string> g_names;
 static uintptr_t g_end;
-static int g_outside, g_launches;
+static int g_outside, g_launches, g_too_large;
 extern "C" {
 void** __hipRegisterFatBinary(const void*) { static void* handle; return &handle; }
 void __hipUnregisterFatBinary(void**) {}
@@ -42,8 +42,9 @@ hipError_t __hipPopCallConfiguration(dim3*, dim3*, size_t*, hipStream_t*) { retu
 hipError_t hipFuncSetAttribute(const void*, hipFuncAttribute, int) { return hipSuccess; }
 hipError_t hipGetDevice(int* device) { *device = 0; return hipSuccess; }
 hipError_t hipGetLastError() { return hipSuccess; }
-hipError_t hipLaunchKernel(const void* kernel, dim3, dim3, void** args, size_t, hipStream_t) {
+hipError_t hipLaunchKernel(const void* kernel, dim3 grid, dim3 block, void** args, size_t, hipStream_t) {
   ++g_launches;
+  g_too_large += (uint64_t)grid.x * block.x > 0xFFFFFFFFull;
   const std::string& name = g_names[kernel];
   auto ends = [](uintptr_t end) { g_outside += end > g_end; };
   if (name.find("mm_small_kernel") != std::string::npos || name.find("mm_join_kernel") != std::string::npos) {
@@ -54,11 +55,11 @@ hipError_t hipLaunchKernel(const void* kernel, dim3, dim3, void** args, size_t, 
   }
   return hipSuccess;
 }
-// -1: a launch wrote past `bytes`; otherwise the call's status.  what: 0 gated_linear, 1 its gradients, 2 int8_bf16
+// -1: a launch wrote past `bytes`, -3: one had more threads than the runtime takes; otherwise the call's status.  what: 0 gated_linear, 1 its gradients, 2 int8_bf16
 int call(int what, const int* splits, int n, long T, long D, long F, size_t bytes) {
   dt::g_splits.assign(splits, splits + n);
   dt::g_read = 0;
-  g_outside = g_launches = 0;
+  g_outside = g_launches = g_too_large = 0;
   uint8_t* const p = reinterpret_cast<uint8_t*>((uintptr_t)1 << 40);
   void* const ws = reinterpret_cast<void*>((uintptr_t)1 << 44);
   g_end = ((uintptr_t)1 << 44) + bytes;
@@ -67,6 +68,7 @@ int call(int what, const int* splits, int n, long T, long D, long F, size_t byte
   else if (what == 1) status = dt_gated_linear_backward(p, p, p, p, p, p, T, D, F, D, D, D, 0, p, p, p, ws, bytes, nullptr);
   else status = dt_int8_bf16(p, p, (const float*)p, (const float*)p, T, F, D, D, D, p, F, ws, bytes, nullptr);
   if (g_outside) return -1;
+  if (g_too_large) return -3;
   return status == 0 && g_launches == 0 ? -2 : status;
 }
 size_t bytes(int what, int splits, long T, long D, long F) {
@@ -110,3 +112,12 @@ def test_all_writes_are_inside(lib, what, size):
             assert status in (0, 5), (given, reads, status)  # done, or the workspace refused
             if len(set(reads)) == 1:
                 assert status == (0 if reads[0] == 1 or given == many else 5)
+
+
+def test_more_threads_than_a_launch_has(lib):
+    """2^24 tiles of 64 rows, 2^32 threads, which the runtime would cut short: an error of the call, and the next call is not affected"""
+    splits = (C.c_int * 1)(1)
+    assert lib.call(2, splits, 1, (1 << 30) - 1, 4, 1, 1 << 62) == 7
+    assert lib.call(2, splits, 1, (1 << 30) - 64, 4, 1, 1 << 62) == 0
+    assert lib.call(0, splits, 1, (1 << 30) - 1, 2, 2, 1 << 62) == 7
+    assert lib.call(0, splits, 1, 100, 64, 64, 1 << 62) == 0
