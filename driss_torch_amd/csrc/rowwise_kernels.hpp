@@ -306,15 +306,28 @@ inline int launch_rowwise_impl(const void* x, int64_t rows, int64_t cols, void* 
   return launch_status();
 }
 
-inline int launch_rowwise(const void* x, int in_dtype, int64_t rows, int64_t cols, int out_dtype, void* out,
-                          float* amax_out, float* scale_out, hipStream_t stream) {
-  if (rows > 0x7FFFFFFFll) return DT_ERR_INVALID_SHAPE;
+inline int launch_rowwise_part(const void* x, int in_dtype, int64_t rows, int64_t cols, int out_dtype, void* out,
+                               float* amax_out, float* scale_out, hipStream_t stream) {
   if (in_dtype == DT_F32) {
     if (out_dtype == DT_E4M3FN) return launch_rowwise_impl<DT_F32, DT_E4M3FN>(x, rows, cols, out, amax_out, scale_out, stream);
     return launch_rowwise_impl<DT_F32, DT_E5M2>(x, rows, cols, out, amax_out, scale_out, stream);
   }
   if (out_dtype == DT_E4M3FN) return launch_rowwise_impl<DT_BF16, DT_E4M3FN>(x, rows, cols, out, amax_out, scale_out, stream);
   return launch_rowwise_impl<DT_BF16, DT_E5M2>(x, rows, cols, out, amax_out, scale_out, stream);
+}
+
+// A launch has fewer than 2^32 threads: as many rows at a time as workgroups may be, from rows on that lie as the first one does
+constexpr int64_t kMostRowsAtOnce = 1 << 23;
+inline int launch_rowwise(const void* x, int in_dtype, int64_t rows, int64_t cols, int out_dtype, void* out,
+                          float* amax_out, float* scale_out, hipStream_t stream) {
+  if (rows > 0x7FFFFFFFll) return DT_ERR_INVALID_SHAPE;
+  for (int64_t row = 0; row < rows; row += kMostRowsAtOnce) {
+    const uint8_t* const from = static_cast<const uint8_t*>(x) + row * cols * (in_dtype == DT_F32 ? 4 : 2);
+    if (const int st = launch_rowwise_part(from, in_dtype, std::min(rows - row, kMostRowsAtOnce), cols, out_dtype, static_cast<uint8_t*>(out) + row * cols,
+                                           amax_out ? amax_out + row : nullptr, scale_out ? scale_out + row : nullptr, stream))
+      return st;
+  }
+  return DT_OK;
 }
 
 }  // namespace dt

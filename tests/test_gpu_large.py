@@ -258,3 +258,17 @@ def test_mx_gemm_output_larger_than_4_gib(d):
     sb_b = co.to_blocked(sb.cpu()).cuda().view(torch.float8_e8m0fnu)
     out = d.mx_fp8_bf16(a.view(E4), b.view(E4).t(), sa_b, sb_b)
     _check_rows(out, [0, 1, 23000, 23048, 46080, M - 2, M - 1], a, sa, b, sb)
+
+
+@pytest.mark.parametrize("rows,cols,in_dtype", [((1 << 26) + 5, 8, torch.bfloat16), ((1 << 24) + 3, 3, torch.float32), ((1 << 24) + 7, 1030, torch.bfloat16)])
+def test_rowwise_more_rows_than_a_launch_has_threads_for(d, rows, cols, in_dtype):
+    period = 1021
+    base = util.normal((period, cols), rows % 1000, in_dtype)
+    x = torch.empty(rows, cols, dtype=in_dtype, device="cuda")
+    whole = rows // period * period
+    x[:whole].view(-1, period, cols).copy_(base.cuda())
+    x[whole:] = base[: rows - whole].cuda()
+    out, amax, scale = d.dynamic_scaled_quant_rowwise(x, E4)
+    for got, want in zip((out.view(torch.uint8), amax.view(rows, 1), scale.view(rows, 1)), co.dynamic_scaled_quant_rowwise(base, E4)):
+        want = want.view(period, -1).cuda()
+        assert bool((got[:whole].view(-1, period, want.shape[1]) == want).all()) and torch.equal(got[whole:], want[: rows - whole])
