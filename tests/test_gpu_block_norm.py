@@ -311,3 +311,11 @@ def test_an_empty_batch_with_its_gate(gpu_device, shape, gate_shape, dtype):
     assert all(g.shape == t.shape and not g.any() for g, t in zip(grads, (r, y, p, w, gate)))
     with pytest.raises(RuntimeError, match="gate must have rows"):
         d.post_norm(torch.zeros(2, 40, dtype=dtype, device=gpu_device), torch.zeros(2, 40, dtype=dtype, device=gpu_device), p, torch.zeros(0, 40, dtype=dtype, device=gpu_device))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,gates", [(2064, 1000, 129), (1290, 4104, 129), (1530, 2056, 255), (774, 9224, 129), (1608, 520, 201), (2056, 521, 257), (1542, 4096, 257), (900, 12288, 300)])
+def test_gate_rows_about_as_many_as_units(gpu_device, rows, cols, gates, dtype):
+    """gate rows of several rows each, one unit to a gate row and several gate rows to a unit"""
+    v = inputs(rows, cols, gates, dtype, rows + cols, gpu_device)
+    check(run(v, "post_pre"), reference(v), (rows, cols, gates))

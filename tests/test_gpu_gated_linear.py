@@ -244,3 +244,21 @@ def test_gradients_where_squares_overflow(gpu_device, t, act):
     want_g, want_u = torch.zeros_like(wg), torch.zeros_like(wu)
     want_g[0, 0], want_g[0, 1], want_u[0, 0], want_u[0, 1] = 2.0**65, 0.5, float("inf"), 2.0**66  # (2^132 is past bf16)
     assert torch.equal(dg, want_g) and torch.equal(du, want_u)
+
+
+# at most 32 rows and more groups of columns than CUs: a workgroup takes several in turn, with rows of whole words and off them, one and two tiles of rows,
+# and few groups of rows off the words with sixteen waves a workgroup
+@pytest.mark.parametrize("t,dim,f", [(1, 256, 14336), (3, 1032, 9001), (8, 130, 16001), (12, 520, 7000), (20, 256, 9000), (32, 64, 20011), (1, 2048, 2731), (3, 129, 9001), (16, 65, 8500),
+                                     (24, 333, 200), (24, 333, 5000), (32, 1001, 4097), (17, 129, 9003), (32, 77, 13000)])
+def test_few_rows_and_many_columns(gpu_device, t, dim, f):
+    act = ACTS[(t + dim + f) % 3]
+    x, wg, wu, _ = inputs(t, dim, f, t + dim + f, gpu_device)
+    want = ref.gated(x, wg, wu, act)
+    h = d.gated_linear(x, wg, wu, act)
+    ref.assert_within(h, *want, (t, dim, f, act))
+    # and with both products kept
+    kept, g, u = d.ops.gated_linear_forward(x, wg, wu, act)
+    assert torch.equal(kept, h)
+    n = dim * 2.0**-24 + ref.E
+    for got, w in ((g, wg), (u, wu)):
+        ref.assert_within(got, ref.f64(x) @ ref.f64(w).t(), n * (ref.f64(x).abs() @ ref.f64(w).abs().t()))

@@ -259,3 +259,10 @@ def test_quantize_many_rows(gpu_device, rows, cols, dtype):
     want, ws = (t.to(gpu_device) for t in quantized(block))
     for got, of in ((q, want), (scale, ws)):
         assert bool((got[:whole].view(-1, period, of.shape[1]) == of).all()) and torch.equal(got[whole:], of[:rows - whole])
+
+
+# at most 32 rows and more groups of columns than CUs: a workgroup takes several in turn, with rows of whole words and off them, one and two tiles of rows
+@pytest.mark.parametrize("m,n,k", [(1, 20000, 512), (1, 66000, 128), (8, 33001, 260), (12, 20000, 1040), (20, 20001, 640), (32, 40000, 132), (5, 9000, 257), (1, 20011, 1001), (16, 8500, 130),
+                                   (24, 9000, 257), (32, 17003, 513), (24, 4000, 333)])
+def test_product_of_few_rows_and_many_columns(gpu_device, m, n, k):
+    check_product(*operands(m, n, k, m + n + k, gpu_device))
