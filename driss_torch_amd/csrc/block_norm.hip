@@ -8,7 +8,7 @@ namespace {
 int norm_args(NormArgs& a, int form, int dtype, int64_t rows, int64_t cols, const void* gate, int64_t gates) {
   if (dtype != DT_F32 && dtype != DT_BF16) return DT_ERR_INVALID_DTYPE;
   if (form < kNormPost || form > kNormPostPre) return DT_ERR_INVALID_MODE;
-  if (rows < 0 || cols < 0 || rows > 0x7FFFFFFFll || cols > 32768) return DT_ERR_INVALID_SHAPE;
+  if (rows < 0 || cols < 0 || rows > 0x7FFFFFFFll || cols > kNormMostCols) return DT_ERR_INVALID_SHAPE;
   if ((gate != nullptr) != (gates > 0) || (gate && form == kNormPre)) return DT_ERR_INVALID_MODE;
   if (gates > 0 && rows % gates) return DT_ERR_INVALID_SHAPE;
   a.rows = rows;

@@ -22,6 +22,7 @@
 
 namespace dt {
 
+constexpr int kNormMostCols = 32768;  // of a row
 enum NormForm { kNormPost = 1, kNormPre = 2, kNormPostPre = 3 };
 
 template <int IN>

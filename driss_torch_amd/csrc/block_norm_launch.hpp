@@ -7,7 +7,9 @@
 
 namespace dt {
 
-constexpr int64_t kNormMostVecs = 8192;  // 16-byte vectors of a row
+// of the longest rows, in sixteen waves
+template <int IN>
+constexpr int kNormMostVecsOfLane = kNormMostCols / NormVec<IN>::kVec / (16 * kWave);
 
 struct NormForwardOut {
   void *new_residual, *normed;
@@ -62,7 +64,7 @@ template <int IN, int FORM>
 int norm_forward_form(const NormArgs& a, const NormForwardOut& out, hipStream_t stream) {
   const bool edges = norm_edges<IN>(a, {out.new_residual, out.normed});
   const int cus = device_facts().cu_count;
-  return norm_team<IN == DT_F32 ? 8 : 4, true>(ceil_div(a.cols, NormVec<IN>::kVec), a.rows <= 2 * cus, [&](auto nv, auto waves) {
+  return norm_team<kNormMostVecsOfLane<IN>, true>(ceil_div(a.cols, NormVec<IN>::kVec), a.rows <= 2 * cus, [&](auto nv, auto waves) {
     constexpr int NV = decltype(nv)::value, WAVES = decltype(waves)::value;
     // as many workgroups as fit the chip at once
     const int64_t fit = (int64_t)cus * std::max(1, 16 / (WAVES == 1 ? 4 : WAVES));
@@ -84,7 +86,7 @@ int norm_backward_form(const NormArgs& a, const NormBackward& b, const NormUnits
   const bool edges = norm_edges<IN>(a, {b.d_new, b.d_normed, b.d_residual, b.d_branch, b.d_gate});
   float* const sums_p = b.sums;
   float* const sums_n = FORM == kNormPostPre ? b.sums + shares.units * a.cols : b.sums;
-  const int status = norm_team<IN == DT_F32 ? 8 : 4, false>(ceil_div(a.cols, NormVec<IN>::kVec), false, [&](auto nv, auto waves) {
+  const int status = norm_team<kNormMostVecsOfLane<IN>, false>(ceil_div(a.cols, NormVec<IN>::kVec), false, [&](auto nv, auto waves) {
     constexpr int NV = decltype(nv)::value, WAVES = decltype(waves)::value;
     const unsigned grid = (unsigned)ceil_div(shares.units, kNormTeams<WAVES>), block = kNormTeams<WAVES> * WAVES * kWave;
     auto launch = [&](auto edges_, auto inside_) {
