@@ -20,7 +20,7 @@ int norm_args(NormArgs& a, int form, int dtype, int64_t rows, int64_t cols, cons
 
 // As many units as fit a CU's registers at once: eight waves, or one workgroup of the longer rows' teams.  With twice as many one half waits for the other
 // and leaves its sums too, cols words a unit written and read again: both norms with all gradients, this many and twice, 2560 x 12288
-// bf16 158 and 176 us, 4096 x 8192 141 and 157, 16384 x 4096 266 and 284, 32768 x 1024 162 and 191.  A unit has four rows at least, but a
+// bf16 154 and 172 us, 4096 x 8192 140 and 154, 16384 x 4096 266 and 285, 32768 x 1024 154 and 183.  A unit has four rows at least, but a
 // chip that would be idle otherwise is given single rows.
 NormUnits norm_units(int dtype, int64_t rows, int64_t cols, int64_t rows_per_gate) {
   const int64_t cus = device_facts().cu_count, gates = rows / rows_per_gate;

@@ -123,12 +123,13 @@ struct NormArgs {
 template <int WAVES>
 constexpr int kNormTeams = WAVES == 1 ? 4 : 1;
 // Whether weights and gate stay in registers and the next row is on its way while this one's sums are joined: a workgroup of sixteen waves has
-// 128 registers a lane, which two vectors of everything else fill (both norms with their gradients, 640 x 11864 bf16: 175 us with both, spilled, 100 without).
+// 128 registers a lane, which two vectors of everything else fill (both norms with their gradients, bf16, with both, spilled, and without: 640 x 16384 112
+// and 91 us, 2560 x 16384 306 and 203).
 template <int NV, int WAVES>
 constexpr bool kNormHold = WAVES < 16 || NV == 1;
 // Whether the sums of the gradients over a unit's rows are in LDS, each word its lane's own: of long rows of bf16, whose eight elements a vector have sixteen
-// sums, the registers hold what comes in instead: gradients of 2560 x 12288, whole pass, 177 us, 203 without and without the next row's loads ahead; with
-// a gate per row 2560 x 9224 169 and 274.
+// sums, the registers hold what comes in instead: both norms with all gradients, sums in LDS and in registers, 2560 x 12288 154 and 269 us, with a gate per
+// row 2560 x 9224 164 and 474, of sixteen waves 2560 x 16384 203 and 241.
 template <int IN, int NV, int WAVES, int FORM>
 constexpr bool kNormSumsInLds = IN == DT_BF16 && FORM == kNormPostPre && ((NV == 3 && WAVES == 8) || (NV == 2 && WAVES == 16));
 template <int IN, int NV, int WAVES, int FORM>
@@ -362,7 +363,7 @@ __global__ __launch_bounds__(kNormTeams<WAVES>* WAVES* kWave) void norm_backward
         raw_y[u] = next_y[u];
       }
     }
-    if (AHEAD && row + 1 < end) fetch(row + 1);
+    if (HOLD && row + 1 < end) fetch(row + 1);
     if constexpr (POST) {
       if (a.gate && gate_row < 0) {
         gate_row = row / a.rows_per_gate;
@@ -376,7 +377,16 @@ __global__ __launch_bounds__(kNormTeams<WAVES>* WAVES* kWave) void norm_backward
         }
       }
     }
-    if constexpr (REBUILD) {
+    // (weights that are not held are asked for at once, in front of the next row's loads, whose registers are free until then)
+    auto build_r = [&]() __attribute__((always_inline)) {
+      u32x4 p_of[HOLD ? 1 : NV], g_of[HOLD ? 1 : NV];
+      if constexpr (!HOLD) {
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+          p_of[u] = Row::template load<false>(a.post_weight, 0, a.cols, t + u * kThreads);
+          g_of[u] = Row::template load<false>(a.gate, gate_row, a.cols, t + u * kThreads);
+        }
+      }
       const float scale = iy * a.scale;
 #pragma unroll
       for (int u = 0; u < NV; ++u) {
@@ -384,8 +394,8 @@ __global__ __launch_bounds__(kNormTeams<WAVES>* WAVES* kWave) void norm_backward
         if (!a.rebuild) continue;
         float y[V::kVec], p[V::kVec], g[V::kVec];
         V::unpack(raw_y[u], y);
-        weight_p(u, p);
-        if (a.gate) gate(u, g);
+        V::unpack(HOLD ? held_p[HOLD ? u : 0] : p_of[HOLD ? 0 : u], p);
+        if (a.gate) V::unpack(HOLD ? held_gate[HOLD ? u : 0] : g_of[HOLD ? 0 : u], g);
 #pragma unroll
         for (int i = 0; i < V::kVec; ++i) {
           float z = y[i] * scale * p[i];
@@ -393,7 +403,9 @@ __global__ __launch_bounds__(kNormTeams<WAVES>* WAVES* kWave) void norm_backward
           r_new[u][i] += z;
         }
       }
-    }
+    };
+    if constexpr (REBUILD) build_r();
+    if (AHEAD && !HOLD && row + 1 < end) fetch(row + 1);
     auto row_r = [&](int u, float (&f)[V::kVec]) __attribute__((always_inline)) {
       if constexpr (REBUILD) {
 #pragma unroll
