@@ -371,7 +371,8 @@ struct BlockNorm : Function<BlockNorm> {
     // of both norms in bf16 the gradients take the new residual as the second norm did, before its rounding, and build it again
     const bool from_residual = branch && pre_weight && residual.scalar_type() == at::kBFloat16;
     ctx->saved_data["from_residual"] = from_residual;
-    ctx->save_for_backward({branch && !from_residual ? new_residual : residual, branch.value_or(none), post_weight.value_or(none), pre_weight.value_or(none), gate.value_or(none), iy, ir});
+    // (those of a norm behind the block alone take only its shape, which is the branch's: its result may change meanwhile)
+    ctx->save_for_backward({!pre_weight ? *branch : branch && !from_residual ? new_residual : residual, branch.value_or(none), post_weight.value_or(none), pre_weight.value_or(none), gate.value_or(none), iy, ir});
     ctx->saved_data["residual_scale"] = residual_scale;
     if (!branch) return {normed};
     if (!pre_weight) return {new_residual};

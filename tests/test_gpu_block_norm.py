@@ -319,3 +319,16 @@ def test_gate_rows_about_as_many_as_units(gpu_device, rows, cols, gates, dtype):
     """gate rows of several rows each, one unit to a gate row and several gate rows to a unit"""
     v = inputs(rows, cols, gates, dtype, rows + cols, gpu_device)
     check(run(v, "post_pre"), reference(v), (rows, cols, gates))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_residual_stream_may_be_added_to_in_place(gpu_device, dtype):
+    """neither the residual nor the result of a norm behind a block is needed for its gradients"""
+    v = inputs(20, 72, 2, dtype, 5, gpu_device, "post")
+    want = run(v, "post")
+    leaves = {**v, **{k: v[k].clone().requires_grad_() for k in ("branch", "post_weight", "gate")}}
+    out = call(leaves, "post")["residual"]
+    out += 1
+    leaves["residual"].zero_()
+    got = torch.autograd.grad(out, [leaves[k] for k in ("branch", "post_weight", "gate")], v["d_residual"])
+    assert all(torch.equal(g, want["d_" + k]) for g, k in zip(got, ("branch", "post_weight", "gate")))
