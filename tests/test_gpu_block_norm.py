@@ -332,3 +332,19 @@ def test_the_residual_stream_may_be_added_to_in_place(gpu_device, dtype):
     leaves["residual"].zero_()
     got = torch.autograd.grad(out, [leaves[k] for k in ("branch", "post_weight", "gate")], v["d_residual"])
     assert all(torch.equal(g, want["d_" + k]) for g, k in zip(got, ("branch", "post_weight", "gate")))
+
+
+def test_offsets_past_32_bits(gpu_device):
+    """a row's values and gradients are the same at the end of tensors of more than 2^31 elements as in tensors of that row's neighbours alone"""
+    rows, cols = 70000, 32760
+    if torch.cuda.mem_get_info()[0] < 64 << 30:
+        pytest.skip("needs 64 GiB of free device memory")
+    g = torch.Generator(device="cuda").manual_seed(0)
+    n = lambda *s: torch.randn(*s, generator=g, device=gpu_device, dtype=torch.bfloat16)  # noqa: E731
+    v = {"residual": n(rows, cols), "branch": n(rows, cols), "post_weight": n(cols), "pre_weight": n(cols), "gate": n(2, cols), "d_residual": n(rows, cols), "d_normed": n(rows, cols)}
+    got = run(v, "post_pre")
+    for part in (slice(0, 40), slice(65560, 65600), slice(rows - 40, rows)):
+        alone = {k: t[part] if t.shape[0] == rows else t for k, t in v.items()}
+        alone["gate"] = v["gate"][0 if part.stop <= rows // 2 else 1]
+        want = run(alone, "post_pre")
+        assert all(torch.equal(got[k][part], want[k]) for k in ("residual", "normed", "d_residual", "d_branch"))

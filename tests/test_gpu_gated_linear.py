@@ -262,3 +262,26 @@ def test_few_rows_and_many_columns(gpu_device, t, dim, f):
     n = dim * 2.0**-24 + ref.E
     for got, w in ((g, wg), (u, wu)):
         ref.assert_within(got, ref.f64(x) @ ref.f64(w).t(), n * (ref.f64(x).abs() @ ref.f64(w).abs().t()))
+
+
+def test_offsets_past_32_bits(gpu_device):
+    """more than 2^31 gated elements: rows at the end as in a call of those rows alone, and weights' gradients of the last rows, the others' being zero"""
+    t, dim, f = 70001, 64, 32760
+    if torch.cuda.mem_get_info()[0] < 96 << 30:
+        pytest.skip("needs 96 GiB of free device memory")
+    g = torch.Generator(device="cuda").manual_seed(0)
+    n = lambda *s: torch.randn(*s, generator=g, device=gpu_device, dtype=torch.bfloat16)  # noqa: E731
+    x, wg, wu = (v.requires_grad_() for v in (n(t, dim), n(f, dim), n(f, dim)))
+    h = d.gated_linear(x, wg, wu)
+    dh = torch.zeros_like(h)
+    last = t - 50
+    dh[last:] = n(50, f)
+    dx, dg, du = torch.autograd.grad(h, (x, wg, wu), dh)
+    for part in (slice(0, 50), slice(65536, 65586), slice(last, t)):
+        ref.assert_within(h[part], *ref.gated(x[part], wg, wu, "silu"), part)
+    assert not dx[:last].any()
+    want = ref.gated_grads(dh[last:], x[last:], wg, wu, "silu")
+    ref.assert_within(dx[last:], *want["dx"], "dx")
+    # (the zero rows add nothing, of however many steps the sum is)
+    ref.assert_within(dg, *want["dw_gate"], "dw_gate")
+    ref.assert_within(du, *want["dw_up"], "dw_up")

@@ -266,3 +266,17 @@ def test_quantize_many_rows(gpu_device, rows, cols, dtype):
                                    (24, 9000, 257), (32, 17003, 513), (24, 4000, 333)])
 def test_product_of_few_rows_and_many_columns(gpu_device, m, n, k):
     check_product(*operands(m, n, k, m + n + k, gpu_device))
+
+
+def test_product_offsets_past_32_bits(gpu_device):
+    """results past element 2^31, and more than 2^32 bytes of either operand; a row's result is the same in a product of fewer"""
+    if torch.cuda.mem_get_info()[0] < 48 << 30:
+        pytest.skip("needs 48 GiB of free device memory")
+    for m, n, k in ((70001, 32760, 64), (70001, 300, 65536), (300, 70001, 65536), (20, 70001, 65536)):
+        a, b = (torch.randint(-127, 128, (r, k), dtype=torch.int8, device=gpu_device) for r in (m, n))
+        sa, sb = (torch.rand(r, 1, device=gpu_device) + 0.01 for r in (m, n))
+        y = d.int8_bf16(a, b.t(), sa, sb)
+        for rows in (slice(0, 17), slice(m - 17, m)):
+            for columns in (slice(0, 40), slice(n - 40, n)):
+                check_product(a[rows], b[columns], sa[rows], sb[columns], y[rows, columns])
+        del a, b, y
