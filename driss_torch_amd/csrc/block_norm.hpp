@@ -13,8 +13,8 @@
 // Every tensor is read once and written once, so memory bounds all of it.  A row stays in the registers of its team of
 // waves between the two sums, both of which are 32 bits wide.  The workgroups are persistent: weights and gate stay in
 // registers from row to row, and the next row's loads are on their way while this one's sums are joined.  16384 x 8192 bf16, both
-// norms: 185 us (5.8 TB/s), gradients 350 us (4.6 TB/s; a row and the sums of a CU fill its registers, so that one row at a time is
-// under way beside the next one's loads) and 8 us for the sums over units; 16 x 8192 4.6 us.
+// norms: 184 us (5.8 TB/s), gradients 332 us (4.9 TB/s; a row and the sums of a CU fill its registers, so that one row at a time is
+// under way beside the next one's loads) and 7 us for the sums over units; 16 x 8192 4.7 us.
 #pragma once
 
 #include "dt_device.hpp"

@@ -1,6 +1,6 @@
 """The operators of a gated feed-forward block between two norms, trained in bf16 and served with 8-bit integer
 products.  A weight has a linear layer's layout, one row per output channel.  ``gated_linear`` and the norms have
-gradients (of first order); everything runs on the current stream of its inputs' device."""
+gradients (of first order, in reverse mode); everything runs on the current stream of its inputs' device."""
 from typing import Optional, Tuple
 
 import torch
@@ -32,8 +32,8 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, activation: str = "sil
     """``act(x @ w_gate.t()) * (x @ w_up.t())`` in bf16, with sums, activation and product in fp32 and one rounding.
 
     x: [..., D]; w_gate, w_up: [F, D]; ``activation``: "silu", "gelu" or "gelu_tanh".  For the gradients both
-    products are kept in fp32; their own gradients are rounded to bf16 before they are multiplied with x and the
-    weights."""
+    products are kept in fp32, 8 bytes an element of the result; their own gradients are rounded to bf16 before they are
+    multiplied with x and the weights."""
     return _ops.gated_linear(x, w_gate, w_up, activation)
 
 
@@ -58,5 +58,6 @@ def post_norm(residual: Tensor, branch: Tensor, weight: Tensor, gate: Optional[T
 def post_pre_norm(residual: Tensor, branch: Tensor, post_weight: Tensor, pre_weight: Tensor, gate: Optional[Tensor] = None,
                   residual_scale: float = 1.0, eps: float = 1e-6) -> Tuple[Tensor, Tensor]:
     """Between two blocks: ``r = post_norm(residual, branch, post_weight, gate, residual_scale, eps)`` and
-    ``pre_norm(r, pre_weight, eps)`` from one pass over the rows, the second from r before its rounding."""
+    ``pre_norm(r, pre_weight, eps)`` from one pass over the rows, the second from r before its rounding, as
+    the gradients take it too.  For those ``residual`` (bf16) or r (fp32) is kept and may not change in place meanwhile."""
     return _ops.post_pre_norm(residual, branch, post_weight, pre_weight, gate, residual_scale, eps)
